@@ -29,13 +29,14 @@ typedef unsigned u2 __attribute__((ext_vector_type(2)));
 // ---- activations ------------------------------------------------------------------------------
 
 // e^x to about an ulp, from the hardware's 2^y: the rounding of x log2(e) is put back as a first-order
-// term. An infinite argument has no such term.
+// term, of either sign. Where 2^y is infinite (from y = 128, x = 88.7) the term would make it NaN, and an
+// infinite x has none: from |y| = 128 on 2^y stays as it is, infinite or, below, zero.
 __device__ __forceinline__ float exponential(float x) {
   const float y = x * 1.44269504f;
   float rest = __builtin_fmaf(x, 1.44269504f, -y);
   rest = __builtin_fmaf(x, 1.92596299e-8f, rest);  // log2(e) - its float32
   const float e = __builtin_amdgcn_exp2f(y);
-  return __builtin_fabsf(y) < 1e4f ? __builtin_fmaf(e, rest * 0.693147181f, e) : e;
+  return __builtin_fabsf(y) < 128.0f ? __builtin_fmaf(e, rest * 0.693147181f, e) : e;
 }
 
 struct Activated {

@@ -398,3 +398,74 @@ def test_refusals() -> None:
         leaves[1].add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         h.sum().backward()
+
+
+def saturating_values(dtype):
+    """g from -1e30 to 1e30, dense where e^-g ends (88.7) and beyond, each value the same in every format."""
+    pieces = [torch.linspace(-200, 200, 1201), torch.linspace(85, 95, 201), torch.linspace(-95, -85, 201)]
+    far = torch.tensor([250.0, 500, 1000, 5000, 6899, 9999, 1e4, 1.1e4, 1e5, 1e10, 1e19, 1e30])
+    values = torch.cat([*pieces, far, -far]).to(dtype).float()
+    bits = values.view(torch.int32) & ~0xFF  # 16 significant bits: exact as two float16 parts
+    return bits.view(torch.float32).to(device="cuda", dtype=dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows, width", [(5, 8), (64, 8), (600, 8), (700, 2048), (4000, 520)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("activation", sorted(ACTIVATIONS))
+def test_saturated_units(activation, dtype, rows, width) -> None:
+    """Finite g from -1e30 to 1e30, one value a feature (x is one in its first column and zero elsewhere, u is
+    one): h, and by the gradients of the gate's bias and weights the slope, are finite and close to float64,
+    in the kernels for few rows, few tiles and the tiles of every format. An activation's relative error
+    grows with |g| 2^-23 in its tail, where it is below 2^-20: 2^-18 of a value and 2^-20 are allowed, and the
+    sums over equal rows at most rows 2^-24 beside it; bfloat16 rounds dg and the results."""
+    require_gpu_extension()
+    show(f"saturated {activation} {dtype} {rows} x {width}")
+    values = saturating_values(dtype)
+    hidden = values.numel()
+    x = torch.zeros(rows, width, device="cuda", dtype=dtype)
+    x[:, 0] = 1
+    gate_weight = torch.zeros(hidden, width, device="cuda", dtype=dtype)
+    gate_weight[:, 0] = values
+    zero, one = torch.zeros(hidden, device="cuda", dtype=dtype), torch.ones(hidden, device="cuda", dtype=dtype)
+    tensors = [leaf(t) for t in (x, gate_weight, torch.zeros_like(gate_weight), zero, one)]
+    h = call(tensors, activation)
+    grads = torch.autograd.grad(h, tensors, torch.ones_like(h))
+    assert all(bool(torch.isfinite(t).all()) for t in (h, *grads))
+    exact = values.double().requires_grad_()
+    h64 = ACTIVATIONS[activation](exact)
+    slope64, = torch.autograd.grad(h64.sum(), exact)
+    rounding = HALF_ULP[BF16] if dtype == BF16 else 0.0
+    relative = 2.0**-18 + rounding
+    assert bool(((h.double() - h64).abs() <= relative * h64.abs() + 2.0**-20).all())
+    # Of the gate's weights: of their first column; x is zero in the others.
+    for got in (grads[3], grads[1][:, 0]):
+        error = (got.double() / rows - slope64).abs()
+        assert bool((error <= (relative + rounding + rows * 2.0**-24) * slope64.abs() + 2.0**-20).all())
+    assert not grads[1][:, 1:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows, width, hidden", [(5, 50, 60), (90, 50, 60), (600, 40, 700), (5000, 520, 1100)])
+def test_non_finite_operands_leave_nothing_finite(dtype, rows, width, hidden) -> None:
+    """A NaN or infinite value of x makes the whole of its row of h and of the input's gradient non-finite,
+    and leaves every other row of both bitwise alone."""
+    require_gpu_extension()
+    show(f"non-finite row {dtype} {rows}")
+    tensors = inputs(rows, width, hidden, dtype, seed=12)
+    upstream = normal(rows, hidden, seed=13, dtype=dtype)
+
+    def run(x):
+        x = leaf(x)
+        h = call([x, *tensors[1:]], "silu")
+        return h.detach(), torch.autograd.grad(h, x, upstream)[0]
+
+    clean = run(tensors[0])
+    others = [r for r in range(rows) if r != 2]
+    for value in (math.nan, math.inf, -math.inf):
+        x = tensors[0].clone()
+        x[2, 7] = value
+        for got, want in zip(run(x), clean):
+            assert not torch.isfinite(got[2]).any()
+            assert torch.equal(got[others], want[others])
