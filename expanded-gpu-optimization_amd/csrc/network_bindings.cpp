@@ -64,6 +64,17 @@ void check_once(const char* what) {
               " is differentiable once: create_graph=True is not supported");
 }
 
+// Forward-mode automatic differentiation has to be an error as well: the kernels read a dual tensor's
+// values alone, and what they write would carry no tangent, a derivative of zero to what follows.
+void check_no_tangent(std::initializer_list<const Tensor*> tensors, const char* what) {
+  for (const Tensor* t : tensors) {
+    TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(/*level=*/0).defined(), what,
+                " has no forward-mode derivative: a dual tensor is not supported");
+  }
+}
+
+const Tensor* maybe(const OptionalTensor& t) { return t.has_value() ? &*t : nullptr; }
+
 // ---- gated linear -------------------------------------------------------------------------------
 
 int activation_of(const std::string& name) {
@@ -158,8 +169,6 @@ bool needs_grad(std::initializer_list<const Tensor*> tensors) {
   return false;
 }
 
-const Tensor* maybe(const OptionalTensor& t) { return t.has_value() ? &*t : nullptr; }
-
 Tensor gated_linear(const Tensor& x, const Tensor& gate_weight, const Tensor& up_weight,
                     const OptionalTensor& gate_bias, const OptionalTensor& up_bias,
                     const std::string& activation) {
@@ -173,6 +182,7 @@ Tensor gated_linear(const Tensor& x, const Tensor& gate_weight, const Tensor& up
   TORCH_CHECK(up_weight.sizes() == gate_weight.sizes(), "up_weight must have gate_weight's shape");
   check_vector(gate_bias, gate_weight.size(0), x, "gate_bias", "x");
   check_vector(up_bias, gate_weight.size(0), x, "up_bias", "x");
+  check_no_tangent({&x, &gate_weight, &up_weight, maybe(gate_bias), maybe(up_bias)}, "gated_linear");
   const bool save = needs_grad({&x, &gate_weight, &up_weight, maybe(gate_bias), maybe(up_bias)});
   if (!save) return GatedLinear::forward(nullptr, x, gate_weight, up_weight, gate_bias, up_bias, kind);
   return GatedLinear::apply(x, gate_weight, up_weight, gate_bias, up_bias, kind);
@@ -309,6 +319,8 @@ variable_list residual_norm(const Tensor& residual, const OptionalTensor& block,
     check_like(*gate, residual, "gate", "residual");
     rows_per_gate(residual, *gate);
   }
+  check_no_tangent({&residual, maybe(block), maybe(gate), &weight, maybe(bias), maybe(post_weight), maybe(post_bias)},
+                   "residual_norm");
   const bool save = needs_grad({&residual, maybe(block), maybe(gate), &weight, maybe(bias), maybe(post_weight),
                                 maybe(post_bias)});
   variable_list out =
@@ -349,6 +361,7 @@ void adamw_step(const std::vector<Tensor>& parameters, const std::vector<Optiona
     const int dtype = dtype_of(p, "parameters");
     TORCH_CHECK(p.is_contiguous(), "parameters must be contiguous (parameter ", k, ")");
     TORCH_CHECK(p.device() == parameters[0].device(), "parameters must be on one device");
+    check_no_tangent({&p, maybe(gradients[k])}, "adamw_step");
     const int64_t numel = p.numel();
     if (gradients[k].has_value()) {
       const Tensor& g = *gradients[k];

@@ -125,8 +125,8 @@ def gated_linear(
     projections, the activation (``"silu"``, ``"tanh"``, ``"gelu"``, ``"sigmoid"``) and the product
     in one gfx950 kernel.
 
-    Differentiable once in every tensor, with gradients that are bitwise reproducible; for the
-    backward it keeps both projections in float32. float32 products have float32 precision (errors
+    Differentiable once in every tensor, in reverse mode, with gradients that are bitwise reproducible;
+    for the backward it keeps both projections in float32. float32 products have float32 precision (errors
     of 2^-23 of an operand's value, or in the larger layers 2^-51 of the largest one in its row along
     the contraction if that is more), and a non-finite operand makes what is formed from it
     non-finite (NaN where float32 arithmetic could give an infinity).
@@ -159,8 +159,8 @@ def residual_norm(
     for each channel, ``[samples, 1, width]`` for each of several problems, or the residual's own
     shape. Without a block, ``(residual, norm(residual) * weight + bias)``.
 
-    Differentiable once in every tensor, with gradients that are bitwise reproducible; sums and
-    statistics are float32, and ``normed`` is formed from ``hidden`` before its rounding.
+    Differentiable once in every tensor, in reverse mode, with gradients that are bitwise reproducible;
+    sums and statistics are float32, and ``normed`` is formed from ``hidden`` before its rounding.
     """
     hidden, normed = load_extension().residual_norm(
         residual, block, gate, weight, bias, post_weight, post_bias, float(residual_scale), kind, float(eps)

@@ -496,3 +496,22 @@ def test_refusals() -> None:
     step([p], [None], m, v, steps, lr=1e-3)
     assert torch.equal(p, p0) and not steps.any()
     step([], [], m, v, steps, lr=1e-3)
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused() -> None:
+    """A parameter or gradient with a tangent raises before anything is changed: the update would leave the
+    parameter's tangent as it was."""
+    from torch.autograd import forward_ad
+
+    require_gpu_extension()
+    show("adamw dual tensors")
+    p, g = normal(300, seed=0), normal(300, seed=1)
+    moments = [torch.zeros(512, device="cuda") for _ in range(2)]
+    steps = torch.zeros(1, dtype=torch.int32, device="cuda")
+    p0 = p.clone()
+    with forward_ad.dual_level():
+        for parameter, gradient in ((forward_ad.make_dual(p, g), g), (p, forward_ad.make_dual(g, p))):
+            with pytest.raises(RuntimeError, match="adamw_step has no forward-mode derivative"):
+                fused_hoad.adamw_step([parameter], [gradient], *moments, steps, lr=1e-3)
+    assert torch.equal(p, p0) and not steps.any() and not moments[0].any()

@@ -469,3 +469,24 @@ def test_non_finite_operands_leave_nothing_finite(dtype, rows, width, hidden) ->
         for got, want in zip(run(x), clean):
             assert not torch.isfinite(got[2]).any()
             assert torch.equal(got[others], want[others])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("needs_grad", [False, True])
+def test_forward_mode_is_refused(needs_grad) -> None:
+    """A dual tensor in any place raises, with and without gradient mode, instead of losing its tangent;
+    the tensors that lie in it are taken as before."""
+    from torch.autograd import forward_ad
+
+    require_gpu_extension()
+    show("gated_linear dual tensors")
+    tensors = inputs(4, 8, 6, F32)
+    plain = call(tensors, "silu")
+    with forward_ad.dual_level(), torch.set_grad_enabled(needs_grad):
+        for k, t in enumerate(tensors):
+            some = list(tensors)
+            some[k] = forward_ad.make_dual(leaf(t) if needs_grad else t, torch.ones_like(t))
+            with pytest.raises(RuntimeError, match="gated_linear has no forward-mode derivative"):
+                call(some, "silu")
+            some[k] = forward_ad.unpack_dual(some[k]).primal
+            assert torch.equal(call(some, "silu"), plain)

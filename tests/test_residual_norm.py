@@ -346,3 +346,26 @@ def test_refusals() -> None:
     leaves = [leaf(x), leaf(w)]
     with pytest.raises(RuntimeError, match="differentiable once"):
         torch.autograd.grad(norm(leaves[0], weight=leaves[1])[1].sum(), leaves[0], create_graph=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("needs_grad", [False, True])
+def test_forward_mode_is_refused(needs_grad) -> None:
+    """A dual tensor in any place raises, with and without gradient mode, instead of losing its tangent;
+    the tensors that lie in it are taken as before."""
+    from torch.autograd import forward_ad
+
+    require_gpu_extension()
+    show("residual_norm dual tensors")
+    t = inputs((4, 8), F32, "layer", (8,), True, True, 3)
+    plain = call(t, kind="layer")
+    with forward_ad.dual_level(), torch.set_grad_enabled(needs_grad):
+        for name, value in t.items():
+            dual = forward_ad.make_dual(leaf(value) if needs_grad else value, torch.ones_like(value))
+            with pytest.raises(RuntimeError, match="residual_norm has no forward-mode derivative"):
+                call({**t, name: dual}, kind="layer")
+            outputs = call({**t, name: forward_ad.unpack_dual(dual).primal}, kind="layer")
+            assert all(torch.equal(a, b) for a, b in zip(outputs, plain))
+        dual = forward_ad.make_dual(t["residual"], torch.ones_like(t["residual"]))
+        with pytest.raises(RuntimeError, match="residual_norm has no forward-mode derivative"):
+            fused_hoad.residual_norm(dual, weight=t["weight"])
