@@ -6,6 +6,7 @@
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <string>
 #include <vector>
@@ -71,6 +72,11 @@ void check_no_tangent(std::initializer_list<const Tensor*> tensors, const char* 
     TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(/*level=*/0).defined(), what,
                 " has no forward-mode derivative: a dual tensor is not supported");
   }
+}
+
+// A trace would hold the allocations of a call and not its kernels, and replay uninitialised memory.
+void check_not_traced(const char* what) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " cannot be recorded by torch.jit.trace");
 }
 
 const Tensor* maybe(const OptionalTensor& t) { return t.has_value() ? &*t : nullptr; }
@@ -172,6 +178,7 @@ bool needs_grad(std::initializer_list<const Tensor*> tensors) {
 Tensor gated_linear(const Tensor& x, const Tensor& gate_weight, const Tensor& up_weight,
                     const OptionalTensor& gate_bias, const OptionalTensor& up_bias,
                     const std::string& activation) {
+  check_not_traced("gated_linear");
   const int64_t kind = activation_of(activation);
   dtype_of(x, "x");
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "x must have shape [..., width] with width > 0");
@@ -297,6 +304,7 @@ variable_list residual_norm(const Tensor& residual, const OptionalTensor& block,
                             const Tensor& weight, const OptionalTensor& bias, const OptionalTensor& post_weight,
                             const OptionalTensor& post_bias, double residual_scale, const std::string& kind,
                             double eps) {
+  check_not_traced("residual_norm");
   const int64_t norm = norm_of(kind);
   dtype_of(residual, "residual");
   TORCH_CHECK(residual.dim() >= 1 && residual.size(-1) > 0, "residual must have shape [..., width] with width > 0");
@@ -346,6 +354,7 @@ void adamw_step(const std::vector<Tensor>& parameters, const std::vector<Optiona
                 const Tensor& exp_avg, const Tensor& exp_avg_sq, const Tensor& steps, double lr, double beta1,
                 double beta2, double eps, double weight_decay, const OptionalTensor& exp_avg_scale,
                 const OptionalTensor& exp_avg_sq_scale, int64_t seed) {
+  check_not_traced("adamw_step");
   TORCH_CHECK(parameters.size() == gradients.size(), "parameters and gradients must be as many");
   TORCH_CHECK(lr >= 0.0 && eps >= 0.0 && weight_decay >= 0.0, "lr, eps and weight_decay must be non-negative");
   TORCH_CHECK(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "the betas must lie in [0, 1)");
@@ -406,6 +415,7 @@ void adamw_step(const std::vector<Tensor>& parameters, const std::vector<Optiona
 
 std::vector<Tensor> decode_moments(const Tensor& exp_avg, const Tensor& exp_avg_sq, const Tensor& exp_avg_scale,
                                    const Tensor& exp_avg_sq_scale) {
+  check_not_traced("decode_moments");
   const int64_t count = exp_avg.numel();
   TORCH_CHECK(count % FHOAD_ADAMW_BLOCK == 0, "packed states hold a multiple of ", FHOAD_ADAMW_BLOCK, " values");
   check_state(exp_avg, torch::kUInt8, count, exp_avg, "exp_avg");
