@@ -490,3 +490,49 @@ def test_forward_mode_is_refused(needs_grad) -> None:
                 call(some, "silu")
             some[k] = forward_ad.unpack_dual(some[k]).primal
             assert torch.equal(call(some, "silu"), plain)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows, width, hidden", [(5, 40, 70), (64, 40, 70), (600, 40, 700), (700, 2048, 300),
+                                                 (4000, 520, 1700)])
+def test_the_largest_float32_values(rows, width, hidden) -> None:
+    """Operands next to the largest float32 value, which bfloat16 rounds to infinity, with others that make
+    up for them: h, the input's gradient and the up weights' gradient element by element. The gate is
+    tanh(30), one, so the products are u = x Wu^T, dx = dh Wu and dWu = dh^T x, whose sums of n products
+    have at most 8 roundings for every 16 of them, 2^-23 each of the sum of magnitudes. The matrix cores
+    take bfloat16 parts below 2^-126 as zero, which changes an operand by at most 2^-126 + 2^-134: that much of
+    each operand's values counts beside it."""
+    require_gpu_extension()
+    show(f"largest values {rows} x {width} x {hidden}")
+    largest = torch.finfo(F32).max
+    edges = [largest, -largest, float.fromhex("0x1.FFp127"), -float.fromhex("0x1.FEFFFEp127"),
+             float.fromhex("0x1.FEp127")]
+
+    def with_edges(t):
+        for k, value in enumerate(edges):
+            t[k, 3 * k + 1] = value
+        return t
+
+    gate_bias = torch.full((hidden,), 30.0, device="cuda")
+    small = 2.0**-115
+
+    def run(x, up_weight, upstream):
+        x, up_weight = leaf(x), leaf(up_weight)
+        h = fused_hoad.gated_linear(x, torch.zeros_like(up_weight), up_weight, gate_bias, activation="tanh")
+        return h.detach(), *torch.autograd.grad(h, (x, up_weight), upstream)
+
+    def close(got, a, b):
+        """got = a b, element by element."""
+        a, b = a.double(), b.double()
+        gamma = (8 * math.ceil(a.shape[1] / 16) + 8) * 2.0**-23
+        lost = (2.0**-126 + 2.0**-134) * (a.abs().sum(1, keepdim=True) + b.abs().sum(0, keepdim=True))
+        assert bool(((got.double() - a @ b).abs() <= gamma * (a.abs() @ b.abs()) + lost).all())
+
+    x, w = normal(rows, width, seed=1), normal(hidden, width, seed=2)
+    upstream = normal(rows, hidden, seed=3)
+    close(run(with_edges(x.clone()), w * small, upstream)[0], with_edges(x.clone()), w.t() * small)
+    close(run(x * small, with_edges(w.clone()), upstream)[0], x * small, with_edges(w.clone()).t())
+    close(run(x * small, w * small, with_edges(upstream.clone()))[1], with_edges(upstream.clone()), w * small)
+    close(run(x * small, with_edges(w.clone()), upstream * small)[1], upstream * small, with_edges(w.clone()))
+    close(run(x * small, w * small, with_edges(upstream.clone()))[2], with_edges(upstream.clone()).t(), x * small)
+    close(run(with_edges(x.clone()), w * small, upstream * small)[2], upstream.t() * small, with_edges(x.clone()))
