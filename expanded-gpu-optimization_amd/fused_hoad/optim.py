@@ -38,7 +38,9 @@ class FusedAdamW(torch.optim.Optimizer):
     formed in float32 and rounded once. A parameter without a gradient is left alone and its step
     not counted. The step counts live on the device and nothing synchronises, so a step can be
     captured in a HIP graph (after a first step, which allocates the state; the options of the group
-    are then those of the capture).
+    are then those of the capture). ``load_state_dict`` writes into the state that is there, and a captured
+    step goes on from what was loaded; only with other ``state_bits`` or on another device the state is a new
+    one, and a step has to be captured again.
 
     The moments of a group are packed in a few tensors; ``state[p]`` holds views of them
     (``exp_avg`` and ``exp_avg_sq`` in ``p``'s shape, or in 8 bits the blocks' codes and their
@@ -81,15 +83,16 @@ class FusedAdamW(torch.optim.Optimizer):
         """Group ``index``'s packed state; made, and filled from ``self.state`` where that has entries,
         when there is none yet (a new group, or a copied optimizer)."""
         if index not in self._packs:
-            packed, views = self._pack(self.param_groups[index], self.state)
+            group = self.param_groups[index]
+            packed, views = self._pack(group)
+            self._fill(group, views, self.state)
             self._packs[index] = packed
             self.state.update(views)
         return self._packs[index]
 
     @staticmethod
-    def _pack(group: dict, states) -> tuple[dict[str, Tensor | None], dict[Tensor, dict[str, Tensor]]]:
-        """A packed state for the group, with the values that ``states`` has, and its views by
-        parameter."""
+    def _pack(group: dict) -> tuple[dict[str, Tensor | None], dict[Tensor, dict[str, Tensor]]]:
+        """A packed state of zeros for the group, and its views by parameter."""
         params, eight = group["params"], group["state_bits"] == 8
         device = params[0].device
         if any(p.device != device for p in params):
@@ -103,6 +106,12 @@ class FusedAdamW(torch.optim.Optimizer):
             "exp_avg_scale": torch.zeros(size // STATE_BLOCK, device=device) if eight else None,
             "exp_avg_sq_scale": torch.zeros(size // STATE_BLOCK, device=device) if eight else None,
         }
+        return packed, FusedAdamW._views(params, packed)
+
+    @staticmethod
+    def _views(params: list[Tensor], packed: dict[str, Tensor | None]) -> dict[Tensor, dict[str, Tensor]]:
+        """What of a packed state belongs to each parameter."""
+        eight = packed["exp_avg_scale"] is not None
         every: dict[Tensor, dict[str, Tensor]] = {}
         at = 0
         for k, p in enumerate(params):
@@ -114,15 +123,32 @@ class FusedAdamW(torch.optim.Optimizer):
                 if eight:
                     scales = packed[name + "_scale"]
                     views[name + "_scale"] = scales[at // STATE_BLOCK : (at + span) // STATE_BLOCK]
+            at += span
+        return every
+
+    @staticmethod
+    def _check(group: dict, every: dict[Tensor, dict[str, Tensor]], states) -> None:
+        """Raises unless each parameter's views take what ``states`` has for it."""
+        for p, views in every.items():
             for name, value in states.get(p, {}).items():
                 if name not in views or views[name].shape != value.shape or (
                     name != "step" and views[name].dtype != value.dtype
                 ):
                     raise ValueError(f"state {name!r} does not fit a parameter of shape {tuple(p.shape)} "
                                      f"with {group['state_bits']}-bit moments")
-                views[name].copy_(value)
-            at += span
-        return packed, every
+
+    @classmethod
+    @torch.no_grad()
+    def _fill(cls, group: dict, every: dict[Tensor, dict[str, Tensor]], states) -> None:
+        """Writes into each parameter's views what ``states`` has for it, and zeros what it has not."""
+        cls._check(group, every, states)
+        for p, views in every.items():
+            given = states.get(p, {})
+            for name, view in views.items():
+                if name in given:
+                    view.copy_(given[name])
+                else:
+                    view.zero_()
 
     @torch.no_grad()
     def step(self, closure: Callable[[], Tensor] | None = None) -> Tensor | None:
@@ -153,24 +179,44 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict: dict) -> None:
         """Options and state of ``state_dict``, whose groups must match this optimizer's. The values
-        are copied into a new packed state with their own types (the base class would cast the
-        moments to the parameters' type)."""
+        are copied into the packed state with their own types (the base class would cast the moments to
+        the parameters' type): into the present one where it has the same layout, else into a new one.
+        Nothing is changed when something does not fit."""
         saved = state_dict["param_groups"]
         if [len(g["params"]) for g in saved] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("the state's parameter groups do not match the optimizer's")
-        merged, packs, views = [], {}, {}
+        merged, packs, fills = [], {}, []
         for index, (group, other) in enumerate(zip(self.param_groups, saved, strict=True)):
             merged.append({**group, **other, "params": group["params"]})
-            if group["params"]:
-                states = {p: state_dict["state"].get(key, {})
-                          for p, key in zip(group["params"], other["params"], strict=True)}
-                packs[index], more = self._pack(merged[-1], states)
-                views.update(more)
+            if not group["params"]:
+                continue
+            states = {p: state_dict["state"].get(key, {})
+                      for p, key in zip(group["params"], other["params"], strict=True)}
+            present = self._packs.get(index)
+            if present is not None and self._same_layout(present, merged[-1]):
+                packs[index], views = present, self._views(group["params"], present)
+            else:
+                packs[index], views = self._pack(merged[-1])
+            self._check(merged[-1], views, states)
+            fills.append((merged[-1], views, states))
+        for fill in fills:
+            self._fill(*fill)
         for group, options in zip(self.param_groups, merged, strict=True):
             group.update(options)
         self._packs = packs
         self.state.clear()
-        self.state.update(views)
+        for _, views, _ in fills:
+            self.state.update(views)
+
+    @staticmethod
+    def _same_layout(packed: dict[str, Tensor | None], group: dict) -> bool:
+        moment = packed["exp_avg"]
+        return (
+            (moment.dtype == torch.uint8) == (group["state_bits"] == 8)
+            and all(p.device == moment.device for p in group["params"])
+            and moment.numel() == packed_state_size(group["params"])
+            and packed["step"].numel() == len(group["params"])
+        )
 
     def moments(self, parameter: Tensor) -> tuple[Tensor, Tensor]:
         """``parameter``'s first and second moments in float32 and its shape."""

@@ -515,3 +515,72 @@ def test_forward_mode_is_refused() -> None:
             with pytest.raises(RuntimeError, match="adamw_step has no forward-mode derivative"):
                 fused_hoad.adamw_step([parameter], [gradient], *moments, steps, lr=1e-3)
     assert torch.equal(p, p0) and not steps.any() and not moments[0].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_step_goes_on_from_a_loaded_state(bits) -> None:
+    """A step is captured, a state of an earlier time is loaded, and the graph's replays go on from it
+    bitwise as eager steps of another optimizer do that loaded the same; the optimizer's own state, loaded
+    into itself, changes nothing; a state that does not fit leaves everything as it was."""
+    require_gpu_extension()
+    show(f"adamw load and replay {bits}")
+    shapes = [(64, 33), (500,)]
+    start = tensors_of(shapes, F32)
+
+    def build():
+        parameters = [torch.nn.Parameter(p.clone()) for p in start]
+        for p in parameters:
+            p.grad = torch.zeros_like(p)
+        return parameters, fused_hoad.FusedAdamW(parameters, state_bits=bits, seed=8, **OPTIONS)
+
+    def feed(parameters, step):
+        for p, g in zip(parameters, tensors_of(shapes, F32, seed=10 * step)):
+            p.grad.copy_(g)
+
+    parameters, optimizer = build()
+    feed(parameters, 1)
+    optimizer.step()
+    saved, then = copy.deepcopy(optimizer.state_dict()), [p.detach().clone() for p in parameters]
+    held = {name: t.data_ptr() for name, t in state_of(optimizer).items() if t is not None}
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        optimizer.step()
+    for step in (2, 3):
+        feed(parameters, step)
+        graph.replay()
+    torch.cuda.synchronize()
+    before = copy.deepcopy(optimizer.state_dict())
+    optimizer.load_state_dict(optimizer.state_dict())
+    bad = copy.deepcopy(saved)
+    bad["state"][1]["exp_avg"] = bad["state"][1]["exp_avg"][:-1]
+    with pytest.raises(ValueError, match="does not fit"):
+        optimizer.load_state_dict(bad)
+    for k, entry in optimizer.state_dict()["state"].items():
+        for name, value in entry.items():
+            assert torch.equal(value, before["state"][k][name]), (k, name)
+
+    def load(parameters, optimizer):
+        optimizer.load_state_dict(saved)
+        with torch.no_grad():
+            for p, value in zip(parameters, then):
+                p.copy_(value)
+
+    load(parameters, optimizer)
+    assert held == {name: t.data_ptr() for name, t in state_of(optimizer).items() if t is not None}
+    others, eager = build()
+    load(others, eager)
+    for step in range(4, 8):
+        feed(parameters, step)
+        graph.replay()
+        torch.cuda.synchronize()
+        feed(others, step)
+        eager.step()
+        assert all(torch.equal(a, b) for a, b in zip(parameters, others)), step
+    for p, q in zip(parameters, others):
+        assert all(torch.equal(a, b) for a, b in zip(optimizer.moments(p), eager.moments(q)))
+    assert bool((state_of(optimizer)["step"] == 5).all())
+    # A state without entries is one of zeros, in place as well.
+    optimizer.load_state_dict({**saved, "state": {}})
+    assert held["exp_avg"] == state_of(optimizer)["exp_avg"].data_ptr()
+    assert all(not t.any() for t in state_of(optimizer).values() if t is not None)
