@@ -4,11 +4,13 @@ from __future__ import annotations
 
 import math
 from collections.abc import Callable, Iterable
+from itertools import chain
+from operator import is_
 
 import torch
 from torch import Tensor
 
-from fused_hoad._extension import adamw_step
+from fused_hoad._extension import adamw_step, load_extension
 
 #: Values of packed state that share a scale; every tensor's state starts at a multiple of it.
 STATE_BLOCK = 256
@@ -45,7 +47,8 @@ class FusedAdamW(torch.optim.Optimizer):
     The moments of a group are packed in a few tensors; ``state[p]`` holds views of them
     (``exp_avg`` and ``exp_avg_sq`` in ``p``'s shape, or in 8 bits the blocks' codes and their
     ``exp_avg_scale`` and ``exp_avg_sq_scale``; ``step``, int32), so ``state_dict`` and
-    ``load_state_dict`` work as usual.
+    ``load_state_dict`` work as usual. What ``state`` and the groups hold counts: entries that were taken out
+    start again from zero, and tensors that were put in place of the views are copied in.
     """
 
     def __init__(
@@ -74,21 +77,45 @@ class FusedAdamW(torch.optim.Optimizer):
         )
 
         self._packs: dict[int, dict[str, Tensor | None]] = {}
+        self._members: dict[int, list[Tensor]] = {}  # the parameters of each
+        self._seen: list[Tensor] = []
 
     def __setstate__(self, state: dict) -> None:
         super().__setstate__(state)
-        self._packs = {}  # made again from self.state
+        self._packs, self._members, self._seen = {}, {}, []  # made again from self.state
 
-    def _packed(self, index: int) -> dict[str, Tensor | None]:
-        """Group ``index``'s packed state; made, and filled from ``self.state`` where that has entries,
-        when there is none yet (a new group, or a copied optimizer)."""
-        if index not in self._packs:
-            group = self.param_groups[index]
-            packed, views = self._pack(group)
-            self._fill(group, views, self.state)
-            self._packs[index] = packed
-            self.state.update(views)
-        return self._packs[index]
+    def _tensors(self) -> list[Tensor]:
+        """The groups' parameters and what ``self.state`` holds."""
+        return [*chain.from_iterable(group["params"] for group in self.param_groups),
+                *chain.from_iterable(map(dict.values, self.state.values()))]
+
+    def _update_packs(self) -> None:
+        """Packs the groups' state where it is not the one of the last step: a first step, a new group, a
+        copied optimizer, parameters or state that were changed from outside. Values come from ``self.state``;
+        the packed state of the same parameters is kept."""
+        if load_extension().same_objects([group["params"] for group in self.param_groups], self.state, self._seen):
+            return
+        for index, group in enumerate(self.param_groups):
+            if not group["params"]:
+                continue
+            packed, views = self._present(index, group) or self._pack(group)
+            self._fill(group, views, {p: {name: value for name, value in self.state[p].items() if name in views[p]}
+                                      for p in group["params"]})
+            self._packs[index], self._members[index] = packed, list(group["params"])
+            for p, own in views.items():
+                self.state[p].update(own)
+        self._seen = self._tensors()
+
+    def _present(self, index: int, group: dict):
+        """Group ``index``'s packed state and its views, if it is of these parameters, on their device and has
+        the moments' width that ``group`` asks for; else ``None``."""
+        packed, params = self._packs.get(index), group["params"]
+        if packed is None or len(params) != len(self._members[index]) or not all(map(is_, params, self._members[index])):
+            return None
+        moment = packed["exp_avg"]
+        if (moment.dtype == torch.uint8) != (group["state_bits"] == 8) or any(p.device != moment.device for p in params):
+            return None
+        return packed, self._views(params, packed)
 
     @staticmethod
     def _pack(group: dict) -> tuple[dict[str, Tensor | None], dict[Tensor, dict[str, Tensor]]]:
@@ -157,10 +184,11 @@ class FusedAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        self._update_packs()
         for index, group in enumerate(self.param_groups):
             if not group["params"]:
                 continue
-            packed = self._packed(index)
+            packed = self._packs[index]
             adamw_step(
                 group["params"],
                 [p.grad for p in group["params"]],
@@ -192,11 +220,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 continue
             states = {p: state_dict["state"].get(key, {})
                       for p, key in zip(group["params"], other["params"], strict=True)}
-            present = self._packs.get(index)
-            if present is not None and self._same_layout(present, merged[-1]):
-                packs[index], views = present, self._views(group["params"], present)
-            else:
-                packs[index], views = self._pack(merged[-1])
+            packs[index], views = self._present(index, merged[-1]) or self._pack(merged[-1])
             self._check(merged[-1], views, states)
             fills.append((merged[-1], views, states))
         for fill in fills:
@@ -204,19 +228,11 @@ class FusedAdamW(torch.optim.Optimizer):
         for group, options in zip(self.param_groups, merged, strict=True):
             group.update(options)
         self._packs = packs
+        self._members = {index: list(self.param_groups[index]["params"]) for index in packs}
         self.state.clear()
         for _, views, _ in fills:
             self.state.update(views)
-
-    @staticmethod
-    def _same_layout(packed: dict[str, Tensor | None], group: dict) -> bool:
-        moment = packed["exp_avg"]
-        return (
-            (moment.dtype == torch.uint8) == (group["state_bits"] == 8)
-            and all(p.device == moment.device for p in group["params"])
-            and moment.numel() == packed_state_size(group["params"])
-            and packed["step"].numel() == len(group["params"])
-        )
+        self._seen = self._tensors()
 
     def moments(self, parameter: Tensor) -> tuple[Tensor, Tensor]:
         """``parameter``'s first and second moments in float32 and its shape."""

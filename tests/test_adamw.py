@@ -5,6 +5,7 @@ without bias, state dicts, graphs and refusals."""
 
 from __future__ import annotations
 
+import collections
 import copy
 import math
 
@@ -584,3 +585,79 @@ def test_captured_step_goes_on_from_a_loaded_state(bits) -> None:
     optimizer.load_state_dict({**saved, "state": {}})
     assert held["exp_avg"] == state_of(optimizer)["exp_avg"].data_ptr()
     assert all(not t.any() for t in state_of(optimizer).values() if t is not None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_and_parameters_changed_from_outside(bits) -> None:
+    """After the state was cleared, replaced or partly taken out, after tensors were put in place of the
+    views, and after a group's parameters were changed, a step equals that of a new optimizer whose state
+    was loaded to be the same. What else the user keeps in the state stays there."""
+    require_gpu_extension()
+    show(f"adamw changed state {bits}")
+    shapes = [(40, 9), (300,), (300,)]
+
+    def build(start):
+        parameters = [torch.nn.Parameter(p.detach().clone()) for p in start]
+        return parameters, fused_hoad.FusedAdamW(parameters, state_bits=bits, seed=4, **OPTIONS)
+
+    def advance(parameters, optimizer, step):
+        for k, p in enumerate(parameters):
+            p.grad = normal(*p.shape, seed=10 * step + k)
+        optimizer.step()
+
+    def fresh(entry):
+        return {name: torch.zeros_like(value) for name, value in entry.items()}
+
+    def clear(optimizer, parameters):
+        optimizer.state.clear()
+        return {}
+
+    def replace(optimizer, parameters):
+        optimizer.state = collections.defaultdict(dict)
+        return {}
+
+    def take_out(optimizer, parameters):
+        del optimizer.state[parameters[1]]
+        return {k: v for k, v in optimizer.state_dict()["state"].items() if k != 1}
+
+    def put_in(optimizer, parameters):
+        optimizer.state[parameters[0]] = fresh(optimizer.state[parameters[0]])
+        optimizer.state[parameters[2]]["step"] = torch.tensor(7.0, device="cuda")
+        return optimizer.state_dict()["state"]
+
+    def keep(optimizer, parameters):
+        optimizer.state[parameters[1]]["mine"] = torch.ones(2, device="cuda")
+        return {k: {n: t for n, t in v.items() if n != "mine"} for k, v in optimizer.state_dict()["state"].items()}
+
+    for change in (clear, replace, take_out, put_in, keep):
+        parameters, optimizer = build(tensors_of(shapes, F32))
+        for step in (1, 2):
+            advance(parameters, optimizer, step)
+        state = copy.deepcopy(change(optimizer, parameters))
+        others, other = build(parameters)
+        other.load_state_dict({"state": state, "param_groups": copy.deepcopy(other.state_dict()["param_groups"])})
+        for step in (3, 4):
+            advance(parameters, optimizer, step)
+            advance(others, other, step)
+            assert all(torch.equal(a, b) for a, b in zip(parameters, others)), (change.__name__, step)
+        for a, b in zip(parameters, others):
+            assert torch.equal(optimizer.state[a]["exp_avg"], other.state[b]["exp_avg"]), change.__name__
+            assert torch.equal(optimizer.state[a]["step"], other.state[b]["step"]), change.__name__
+        if change is keep:
+            assert torch.equal(optimizer.state[parameters[1]]["mine"], torch.ones(2, device="cuda"))
+
+    # The last two, of one size, change places; then a new parameter takes the first one's.
+    parameters, optimizer = build(tensors_of(shapes, F32))
+    advance(parameters, optimizer, 1)
+    moments = [[t.clone() for t in optimizer.moments(p)] for p in parameters]
+    group = optimizer.param_groups[0]
+    new = torch.nn.Parameter(normal(40, 9, seed=99))
+    group["params"] = [new, parameters[2], parameters[1]]
+    for p in group["params"]:
+        p.grad = None
+    optimizer.step()
+    for p, want in ((parameters[1], moments[1]), (parameters[2], moments[2])):
+        assert all(torch.equal(a, b) for a, b in zip(optimizer.moments(p), want))
+        assert int(optimizer.state[p]["step"]) == 1
+    assert not optimizer.moments(new)[0].any() and int(optimizer.state[new]["step"]) == 0
