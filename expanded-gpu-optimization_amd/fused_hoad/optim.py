@@ -26,6 +26,23 @@ def packed_state_size(parameters: Iterable[Tensor]) -> int:
     return sum(state_span(p.numel()) for p in parameters)
 
 
+def _check_options(group: dict) -> None:
+    """Raises ``ValueError`` for options that a step does not take or would not heed."""
+    if not group["lr"] >= 0.0 or not group["eps"] >= 0.0 or not group["weight_decay"] >= 0.0:
+        raise ValueError("lr, eps and weight_decay must be non-negative")
+    beta1, beta2 = group["betas"]
+    if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0):
+        raise ValueError("betas must lie in [0, 1)")
+    if group["state_bits"] not in (8, 32):
+        raise ValueError("state_bits must be 8 or 32")
+    if not 0 <= group["seed"] < 2**32:
+        raise ValueError("seed must fit 32 bits")
+    if group.get("amsgrad") or group.get("maximize"):
+        raise ValueError("amsgrad and maximize are not supported")
+    if group["weight_decay"] and not group.get("decoupled_weight_decay", True):
+        raise ValueError("weight_decay that is not decoupled is not supported")
+
+
 class FusedAdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` (decoupled weight decay; no amsgrad, no maximize) as one native call
     a parameter group: two kernels for every 108 tensors, whatever their sizes.
@@ -62,14 +79,6 @@ class FusedAdamW(torch.optim.Optimizer):
         state_bits: int = 32,
         seed: int = 0,
     ) -> None:
-        if not lr >= 0.0 or not eps >= 0.0 or not weight_decay >= 0.0:
-            raise ValueError("lr, eps and weight_decay must be non-negative")
-        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
-            raise ValueError("betas must lie in [0, 1)")
-        if state_bits not in (8, 32):
-            raise ValueError("state_bits must be 8 or 32")
-        if not 0 <= seed < 2**32:
-            raise ValueError("seed must fit 32 bits")
         super().__init__(
             params,
             {"lr": lr, "betas": betas, "eps": eps, "weight_decay": weight_decay,
@@ -79,6 +88,11 @@ class FusedAdamW(torch.optim.Optimizer):
         self._packs: dict[int, dict[str, Tensor | None]] = {}
         self._members: dict[int, list[Tensor]] = {}  # the parameters of each
         self._seen: list[Tensor] = []
+
+    def add_param_group(self, param_group: dict) -> None:
+        """Adds a group, with the defaults for options that it does not give."""
+        _check_options({**self.defaults, **param_group})
+        super().add_param_group(param_group)
 
     def __setstate__(self, state: dict) -> None:
         super().__setstate__(state)
@@ -216,6 +230,7 @@ class FusedAdamW(torch.optim.Optimizer):
         merged, packs, fills = [], {}, []
         for index, (group, other) in enumerate(zip(self.param_groups, saved, strict=True)):
             merged.append({**group, **other, "params": group["params"]})
+            _check_options(merged[-1])
             if not group["params"]:
                 continue
             states = {p: state_dict["state"].get(key, {})

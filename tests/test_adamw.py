@@ -661,3 +661,31 @@ def test_state_and_parameters_changed_from_outside(bits) -> None:
         assert all(torch.equal(a, b) for a, b in zip(optimizer.moments(p), want))
         assert int(optimizer.state[p]["step"]) == 1
     assert not optimizer.moments(new)[0].any() and int(optimizer.state[new]["step"]) == 0
+
+
+def test_options_of_groups_and_of_loaded_states_are_checked() -> None:
+    """As the constructor's: a group's own options, those of a group added later, and those of a state
+    that is loaded, another optimizer's among them, which a step would not heed."""
+    def parameter():
+        return torch.nn.Parameter(torch.zeros(3))
+
+    optimizer = fused_hoad.FusedAdamW([parameter()])
+    for options in ({"lr": -1.0}, {"eps": -1.0}, {"weight_decay": -0.1}, {"betas": (1.0, 0.9)}, {"state_bits": 16},
+                    {"seed": -1}, {"amsgrad": True}, {"maximize": True}, {"decoupled_weight_decay": False}):
+        with pytest.raises(ValueError):
+            fused_hoad.FusedAdamW([{"params": [parameter()], **options}])
+        with pytest.raises(ValueError):
+            optimizer.add_param_group({"params": [parameter()], **options})
+        saved = optimizer.state_dict()
+        saved["param_groups"] = [{**saved["param_groups"][0], **options}]
+        with pytest.raises(ValueError):
+            optimizer.load_state_dict(saved)
+    assert len(optimizer.param_groups) == 1 and optimizer.param_groups[0]["lr"] == 1e-3
+    with pytest.raises(ValueError, match="maximize"):
+        optimizer.load_state_dict(torch.optim.AdamW([parameter()], maximize=True).state_dict())
+    with pytest.raises(ValueError, match="decoupled"):
+        optimizer.load_state_dict(torch.optim.Adam([parameter()], weight_decay=0.1).state_dict())
+    optimizer.load_state_dict(torch.optim.AdamW([parameter()], lr=0.5).state_dict())
+    assert optimizer.param_groups[0]["lr"] == 0.5 and optimizer.param_groups[0]["state_bits"] == 32
+    optimizer.add_param_group({"params": [parameter()], "state_bits": 8})
+    assert optimizer.param_groups[1]["state_bits"] == 8 and optimizer.param_groups[1]["betas"] == (0.9, 0.999)
