@@ -689,3 +689,42 @@ def test_options_of_groups_and_of_loaded_states_are_checked() -> None:
     assert optimizer.param_groups[0]["lr"] == 0.5 and optimizer.param_groups[0]["state_bits"] == 32
     optimizer.add_param_group({"params": [parameter()], "state_bits": 8})
     assert optimizer.param_groups[1]["state_bits"] == 8 and optimizer.param_groups[1]["betas"] == (0.9, 0.999)
+
+
+@pytest.mark.gpu
+def test_last_blocks_of_a_large_tensor() -> None:
+    """70 million equal values and gradients, 8-bit states. After the first step, which the states' rounding
+    does not reach, every parameter is the same and moved; the last blocks' codes, scales and parameters,
+    the one that the tensor ends in among them, equal the elementary form's after both steps."""
+    require_gpu_extension()
+    show("adamw 70M, last blocks")
+    count, last = 70_000_001, 4 * STATE_BLOCK
+    parameter = torch.nn.Parameter(torch.ones(count, device="cuda"))
+    parameter.grad = torch.full((count,), 0.25, device="cuda")
+    optimizer = fused_hoad.FusedAdamW([parameter], state_bits=8, seed=1, **OPTIONS)
+    end = state_span(count)
+    places = torch.arange(end - last, end, device="cuda")
+    inside = places < count
+    beta1, beta2 = OPTIONS["betas"]
+    p = torch.ones(last, device="cuda")
+    g = torch.where(inside, 0.25, 0.0)
+    mean, square = torch.zeros(last, device="cuda"), torch.zeros(last, device="cuda")
+    for step in (1, 2):
+        optimizer.step()
+        size = torch.tensor(OPTIONS["lr"] / (1 - beta1**step), dtype=F32, device="cuda")
+        root = torch.tensor(1 / math.sqrt(1 - beta2**step), dtype=F32, device="cuda")
+        mean = mean * beta1 + g * (1 - beta1)
+        square = square * beta2 + g * g * (1 - beta2)
+        deviation = torch.sqrt(square)
+        p = p * (1 - OPTIONS["lr"] * OPTIONS["weight_decay"]) - size * (mean / (deviation * root + OPTIONS["eps"]))
+        steps = torch.full_like(places, step)
+        random = mix(places ^ mix((steps + mix(torch.full_like(steps, 1))) & 0xFFFFFFFF))
+        codes = encode(mean, random >> 16, 3) + encode(deviation, random & 0xFFFF, 4)
+        pack = state_of(optimizer)
+        for name, want in zip(("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_scale"), codes):
+            assert torch.equal(pack[name][-want.numel():], want), (step, name)
+        there = int(inside.sum())
+        assert torch.equal(parameter.detach()[-there:], p[inside]), step
+        if step == 1:
+            assert bool((parameter.detach() == p[0]).all()) and float(p[0]) < 1.0 - 0.9 * OPTIONS["lr"]
+        mean, square = decode(codes[0], codes[1], 3), decode(codes[2], codes[3], 4) ** 2

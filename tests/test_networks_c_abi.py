@@ -1,6 +1,6 @@
 """The C ABI of libfused_hoad_networks.so (include/fused_hoad_networks.h) through ctypes: every declared
-function is exported, and bad arguments are refused with a status and a message before a device is
-touched."""
+function is exported, bad arguments are refused with a status and a message before a device is
+touched, and on the GPU every call gives bitwise what the Python entry points do."""
 
 from __future__ import annotations
 
@@ -144,3 +144,194 @@ def test_adamw_refusals() -> None:
     assert decode(ptr(P), ptr(0), ptr(P), i64(256), 0, ptr(0)) == INVALID_VALUE
     assert decode(ptr(P + 4), ptr(P), ptr(P), i64(256), 0, ptr(0)) == MISALIGNED
     assert decode(ptr(P), ptr(P), ptr(P), i64(0), 0, ptr(0)) == 0
+
+
+# ---- calls that run kernels: device pointers of torch tensors, the default stream and one of its own ---
+
+
+def address(tensor):
+    return ctypes.c_void_p(None if tensor is None else tensor.data_ptr())
+
+
+def made(lib, status):
+    assert status == 0, lib.fhoad_net_last_error()
+
+
+def streams():
+    import torch
+
+    return (torch.cuda.current_stream(), torch.cuda.Stream())
+
+
+def on(stream):
+    """The stream as an argument, after what the current one has to do yet."""
+    import torch
+
+    stream.wait_stream(torch.cuda.current_stream())
+    return ctypes.c_void_p(stream.cuda_stream)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("rows, width, hidden", [(7, 33, 40), (700, 264, 512), (3000, 700, 1700)])
+def test_gated_linear_runs(rows, width, hidden, dtype) -> None:
+    """Forward with and without the saved values, and backward with all gradients and with some, give bitwise
+    what the Python entry point does, and nothing is written past an output's or the workspace's end."""
+    import torch
+
+    import fused_hoad
+    from gpu_helpers import require_gpu_extension
+    from network_helpers import leaf, normal, show
+
+    require_gpu_extension()
+    show(f"C gated linear {rows} x {width} x {hidden} {dtype}")
+    lib, kind = _lib(), (torch.float32, torch.bfloat16)[dtype]
+    x, gw, uw = normal(rows, width, seed=1, dtype=kind), *(normal(hidden, width, seed=k, dtype=kind, scale=width**-0.5) for k in (2, 3))
+    gb, ub, dh = normal(hidden, seed=4, dtype=kind), normal(hidden, seed=5, dtype=kind), normal(rows, hidden, seed=6, dtype=kind)
+    tensors = [leaf(t) for t in (x, gw, uw, gb, ub)]
+    want = fused_hoad.gated_linear(*tensors, activation="gelu")
+    want_grads = torch.autograd.grad(want, tensors, dh)
+    guard = 64
+
+    def guarded(count, like):
+        return torch.full((count + guard,), 7, dtype=like, device="cuda")
+
+    def whole(buffer, value):
+        assert torch.equal(buffer[:-guard].view(value.shape), value) and bool((buffer[-guard:] == 7).all())
+
+    sizes = (i64(rows), i64(width), i64(hidden))
+    for stream in streams():
+        saved = guarded(lib.fhoad_gated_linear_saved_size(i64(rows), i64(hidden)) // 4, torch.float32)
+        for pre in (saved, None):
+            size = lib.fhoad_gated_linear_forward_workspace_size(*sizes, dtype)
+            h, workspace = guarded(rows * hidden, kind), guarded(size, torch.uint8)
+            made(lib, lib.fhoad_gated_linear_forward(
+                *map(address, (x, gw, uw, gb, ub, h, pre, workspace if size else None)), ctypes.c_size_t(size), *sizes,
+                2, dtype, on(stream)))
+            torch.cuda.synchronize()
+            whole(h, want.detach())
+            assert bool((workspace[size:] == 7).all())
+        assert bool((saved[-guard:] == 7).all())
+        size = lib.fhoad_gated_linear_backward_workspace_size(*sizes, dtype)
+        for asked in ((True,) * 5, (True, False, False, False, True), (False, True, True, True, False)):
+            out = [guarded(g.numel(), kind) if yes else None for g, yes in zip(want_grads, asked)]
+            workspace = guarded(size, torch.uint8)
+            made(lib, lib.fhoad_gated_linear_backward(
+                *map(address, (x, gw, uw, saved, dh, *out, workspace)), ctypes.c_size_t(size), *sizes, 2, dtype, on(stream)))
+            torch.cuda.synchronize()
+            for buffer, grad in zip(out, want_grads):
+                if buffer is not None:
+                    whole(buffer, grad)
+            assert bool((workspace[size:] == 7).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("kind, width", [(0, 96), (1, 1365)])
+def test_residual_norm_runs(kind, width, dtype) -> None:
+    """Forward with and without statistics and hidden, and backward with all gradients and with some, as
+    above; without a block hidden may be left out."""
+    import torch
+
+    import fused_hoad
+    from gpu_helpers import require_gpu_extension
+    from network_helpers import leaf, normal, show
+
+    require_gpu_extension()
+    show(f"C residual norm {kind} {width} {dtype}")
+    lib, like = _lib(), (torch.float32, torch.bfloat16)[dtype]
+    samples, each = 4, 30
+    rows, name = samples * each, ("rms", "layer")[kind]
+    t = {n: leaf(normal(*shape, seed=k, dtype=like)) for k, (n, shape) in enumerate({
+        "residual": (samples, each, width), "block": (samples, each, width), "gate": (samples, 1, width),
+        "weight": (width,), "bias": (width,), "post_weight": (width,), "post_bias": (width,)}.items())}
+    up = [normal(samples, each, width, seed=20 + k, dtype=like) for k in (0, 1)]
+    residual, block, gate, weight, bias, post_weight, post_bias = t.values()
+    want = fused_hoad.residual_norm(residual, block, gate, weight=weight, bias=bias, post_weight=post_weight,
+                                    post_bias=post_bias, residual_scale=1.5, kind=name, eps=1e-5)
+    want_grads = torch.autograd.grad(want, list(t.values()), up)
+    alone = fused_hoad.residual_norm(residual.detach(), weight=weight.detach(), kind=name, eps=1e-5)[1]
+    d = ctypes.c_double
+    for stream in streams():
+        for statistics in (torch.empty(rows, 4, device="cuda"), None):
+            hidden, normed = torch.empty_like(residual), torch.empty_like(residual)
+            made(lib, lib.fhoad_residual_norm_forward(
+                *map(address, (*t.values(), hidden, normed, statistics)), i64(rows), i64(width), i64(each), kind, dtype,
+                d(1.5), d(1e-5), on(stream)))
+            torch.cuda.synchronize()
+            assert torch.equal(hidden, want[0]) and torch.equal(normed, want[1])
+            if statistics is not None:
+                kept = statistics
+        normed = torch.empty_like(residual)
+        made(lib, lib.fhoad_residual_norm_forward(
+            *map(address, (residual, None, None, weight, None, None, None, None, normed, None)), i64(rows), i64(width),
+            i64(rows), kind, dtype, d(1.0), d(1e-5), on(stream)))
+        torch.cuda.synchronize()
+        assert torch.equal(normed, alone)
+        size = lib.fhoad_residual_norm_backward_workspace_size(i64(rows), i64(width), i64(each))
+        for asked in ((True,) * 7, (True, False, True, False, False, False, False), (False, True, False, True, True, True, True)):
+            out = [torch.empty_like(g) if yes else None for g, yes in zip(want_grads, asked)]
+            workspace = torch.full((size + 64,), 7, dtype=torch.uint8, device="cuda")
+            made(lib, lib.fhoad_residual_norm_backward(
+                *map(address, (residual, block, gate, weight, post_weight, post_bias, kept, *up, *out, workspace)),
+                ctypes.c_size_t(size), i64(rows), i64(width), i64(each), kind, dtype, d(1.5), on(stream)))
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want_grads) if a is not None)
+            assert bool((workspace[size:] == 7).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_adamw_runs(dtype, bits) -> None:
+    """Two steps over three tensors, whose state lies in another order than they are given in, and the moments
+    decoded: bitwise those of the Python entry points."""
+    import torch
+
+    import fused_hoad
+    from gpu_helpers import require_gpu_extension
+    from network_helpers import normal, show
+
+    require_gpu_extension()
+    show(f"C adamw {dtype} {bits}")
+    lib, like = _lib(), (torch.float32, torch.bfloat16)[dtype]
+    shapes = [(300,), (7, 11), (5000,)]
+    start = [normal(*s, seed=k, dtype=like) for k, s in enumerate(shapes)]
+    grads = [normal(*s, seed=10 + k, dtype=like) for k, s in enumerate(shapes)]
+    size = fused_hoad.packed_state_size(start)
+    offsets = [0, 512, 768]
+    moment = torch.uint8 if bits == 8 else torch.float32
+    results = []
+    for through_c in (False, True):
+        parameters = [p.clone() for p in start]
+        mean, square = (torch.zeros(size, dtype=moment, device="cuda") for _ in range(2))
+        scales = [torch.zeros(size // 256, device="cuda") for _ in range(2)] if bits == 8 else [None, None]
+        steps = torch.zeros(3, dtype=torch.int32, device="cuda")
+        for _ in range(2):
+            if through_c:
+                order = (2, 0, 1)
+                table = (Tensor * 3)(*[Tensor(parameters[k].data_ptr(), grads[k].data_ptr(), parameters[k].numel(), offsets[k], k)
+                                       for k in order])
+                need = lib.fhoad_adamw_workspace_size(i64(3))
+                workspace = torch.full((need + 64,), 7, dtype=torch.uint8, device="cuda")
+                d = ctypes.c_double
+                made(lib, lib.fhoad_adamw_step(
+                    table, i64(3), dtype, bits, *map(address, (mean, square, *scales, steps, workspace)),
+                    ctypes.c_size_t(need), d(2e-3), d(0.9), d(0.99), d(1e-8), d(0.05), ctypes.c_uint32(9),
+                    on(torch.cuda.Stream())))
+                torch.cuda.synchronize()
+                assert bool((workspace[need:] == 7).all())
+            else:
+                fused_hoad.adamw_step(parameters, grads, mean, square, steps, lr=2e-3, betas=(0.9, 0.99), eps=1e-8,
+                                      weight_decay=0.05, exp_avg_scale=scales[0], exp_avg_sq_scale=scales[1], seed=9)
+        decoded = []
+        if bits == 8:
+            decoded = list(fused_hoad.decode_moments(mean, square, *scales))
+            if through_c:
+                for k, (codes, scale) in enumerate(zip((mean, square), scales)):
+                    out = torch.empty(size, device="cuda")
+                    made(lib, lib.fhoad_adamw_decode(*map(address, (codes, scale, out)), i64(size), k, on(torch.cuda.Stream())))
+                    torch.cuda.synchronize()
+                    assert torch.equal(out, decoded[k])
+        results.append([*parameters, mean, square, steps, *decoded])
+    assert all(torch.equal(a, b) for a, b in zip(*results))

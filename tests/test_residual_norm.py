@@ -369,3 +369,81 @@ def test_forward_mode_is_refused(needs_grad) -> None:
         dual = forward_ad.make_dual(t["residual"], torch.ones_like(t["residual"]))
         with pytest.raises(RuntimeError, match="residual_norm has no forward-mode derivative"):
             fused_hoad.residual_norm(dual, weight=t["weight"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("width", [8201, 10001, 16381])
+@pytest.mark.parametrize("column", [-1, -3, 0])
+def test_infinite_weight_of_wide_rows(column, width, dtype) -> None:
+    """As test_infinite_weight, where a row's values are read again in each pass."""
+    test_infinite_weight(column, width, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("unaligned", [False, True])
+@pytest.mark.parametrize("gate", ["none", "channel", "sample", "element"])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_rows_of_one_value(kind, gate, unaligned, dtype) -> None:
+    """Rows shorter than any vector, element by element against float64, where norms cancel: each rounding
+    counts as 2^-24 of a term, sixteen of them to a value, forty-eight more to a sum over the rows, and in
+    bfloat16 the result's.
+
+    RMS: the gradient through a norm, eps / (x^2 + eps)^(3/2) w dy, is what two terms of about w dy / |x|
+    leave. Layer: a value is its own mean, so a norm gives its bias exactly, and nothing goes back through the
+    first norm. Through the second goes what one rounding of hidden (below 8, formed again in the backward) makes
+    of it at 1 / sqrt(eps) = 1,000: a unit value of u = 1,000 x 2^-20 instead of zero, and by its square and the
+    rounding of w dy 1,000 (u^2 + 2^-23) = 0.00103 of w dy."""
+    require_gpu_extension()
+    show(f"residual_norm one value {kind} {gate} {unaligned} {dtype}")
+    shape = (3, 50, 1)
+    gates = {"none": None, "channel": (1,), "sample": (3, 1, 1), "element": shape}
+    t = inputs(shape, dtype, kind, gates[gate], True, kind == "layer", 5)
+    for name in ("residual", "block"):  # away from zero, where what cancels has no bound
+        t[name] = (t[name].abs().clamp(max=3.0) + 1.0).to(dtype)
+    if unaligned:
+        for name, value in t.items():
+            if value is not None:
+                t[name] = torch.empty(value.numel() + 1, dtype=dtype, device="cuda")[1:].view(value.shape).copy_(value)
+    t = {k: None if v is None else v.requires_grad_(True) for k, v in t.items()}
+    up = [normal(*shape, seed=9, dtype=dtype), normal(*shape, seed=10, dtype=dtype)]
+    outputs = call(t, 1.5, kind)
+    wanted = [k for k in NAMES if t[k] is not None]
+    grads = dict(zip(wanted, torch.autograd.grad(outputs, [t[k] for k in wanted], up)))
+    exact = {k: double(v) for k, v in t.items()}
+    outputs64 = formula(exact, 1.5, kind, 1e-6)
+    grads64 = dict(zip(wanted, torch.autograd.grad(outputs64, [exact[k] for k in wanted], [u.double() for u in up])))
+    rounding = HALF_ULP[BF16] if dtype == BF16 else 0.0
+    one = torch.ones(1, device="cuda", dtype=torch.float64)
+
+    def size(name):
+        return one if exact[name] is None else exact[name].detach().abs()
+
+    def summed(values, like):
+        values = values.expand(shape)
+        return values if like.shape == shape else values.sum((0, 1) if like.dim() == 1 else 1).reshape(like.shape)
+
+    if kind == "layer":
+        assert torch.equal(outputs[1], t["bias"].detach().expand(shape))
+        assert not grads["block"].any() and not grads["post_weight"].any()
+    for got, want in zip(outputs, outputs64):
+        assert bool(((got.double() - want).abs() <= (2.0**-20 + rounding) * want.abs() + 2.0**-20).all())
+    dh, dy = (u.double().abs() for u in up)
+    unit = 1000 * 2.0**-20 if kind == "layer" else 0.0
+    through = 0.00103 * size("weight") * dy if kind == "layer" else 2.0**-20 * size("weight") * dy / outputs64[0].detach().abs()
+    total = dh + size("weight") * dy / (outputs64[0].detach().abs() if kind == "rms" else one)
+    branch = size("post_weight") if kind == "rms" else size("post_bias")
+    bounds = {
+        "residual": 1.5 * (through + 2.0**-20 * dh),
+        "block": 2.0**-20 * size("gate") * total * size("post_weight") / size("block"),
+        "gate": branch * (2.0**-18 * total + through),
+        "weight": (2.0**-18 + unit) * dy * 1.01,
+        "bias": 2.0**-18 * dy,
+        "post_weight": size("gate") * (2.0**-18 * total + through) * 1.01,
+        "post_bias": size("gate") * (2.0**-18 * total + through),
+    }
+    for name in wanted:
+        want = grads64[name]
+        bound = summed(bounds[name], want) + rounding * want.abs()
+        assert bool(((grads[name].double() - want).abs() <= bound).all()), name
