@@ -102,8 +102,8 @@ __device__ __forceinline__ unsigned bf16_pair(float a, float b) {
 }
 
 // The three bf16 parts of two values, each rounded to nearest: x = hi + mid + lo exactly (for
-// |x| from 1e-32 up; below, the low parts are subnormal bf16 values, which the matrix cores take as
-// zero). The 2^15 float32 values next to the largest, which would round to an infinite hi, take the
+// |x| from 1e-32 up; below, parts may be subnormal bf16 values, which the matrix cores take as zero: 2^-126
+// of x at most). The 2^15 float32 values next to the largest, which would round to an infinite hi, take the
 // largest bf16 instead, and their remainders are whole again (this selection takes 1 to 3 % of the time of
 // layers of 256 to 6,000 rows). An infinite value has a NaN remainder: what is formed from it is NaN.
 __device__ __forceinline__ void split_pair(float a, float b, unsigned& hi, unsigned& mid, unsigned& lo) {
@@ -136,9 +136,11 @@ __device__ __forceinline__ void split_half_pair(float a, float b, unsigned& hi, 
 //   Bf16:      bfloat16 values as they are, one product.
 //   Bf16Parts: float32 values as three bf16 parts, six products (the other three are below 2^-24 of
 //              a product). No preparation, every magnitude: the smaller products take it.
-//   HalfParts: float32 values as two float16 parts, three products (the fourth is below 2^-24), hi hi
-//              and the two with a lo in accumulators of their own, 2^11 apart. Half the matrix
-//              instructions, which bound the large products, but float16's range needs each row
+//   HalfParts: float32 values as two float16 parts, three products, hi hi and the two with a lo in
+//              accumulators of their own, 2^11 apart. The fourth, lo lo, is left out: at most 2^-22 of a
+//              product, and that much and of one sign where both values are 1 + 2^-11 (above 2^-24 for 13 %
+//              of uniformly drawn pairs). With the parts' own 2^-23 of each value a product is good to 2^-21,
+//              and a sum to that of its products' magnitudes. Half the matrix instructions, which bound the large products, but float16's range needs each row
 //              scaled by a power of two to its largest value (a pass over the operands first), and
 //              twice the accumulators halve the tile (input gradient at 65,536 x 1,024 x 2,731: 300
 //              TFLOP/s; with lo unscaled and one set of accumulators 366, but then what is a 2^18th of

@@ -126,10 +126,10 @@ def gated_linear(
     in one gfx950 kernel.
 
     Differentiable once in every tensor, in reverse mode, with gradients that are bitwise reproducible;
-    for the backward it keeps both projections in float32. float32 products have float32 precision (errors
-    of 2^-23 of an operand's value, or in the larger layers 2^-51 of the largest one in its row along
-    the contraction if that is more), and a non-finite operand makes what is formed from it
-    non-finite (NaN where float32 arithmetic could give an infinity).
+    for the backward it keeps both projections in float32. float32 products are good to 2^-24 of themselves
+    and 2^-126 of their operands' values; in the larger layers to 2^-21, and to 2^-51 of the largest value in
+    an operand's row along the contraction. A non-finite operand makes the projections and gradients formed
+    from it non-finite (NaN where float32 arithmetic could give an infinity).
     """
     return load_extension().gated_linear(x, gate_weight, up_weight, gate_bias, up_bias, activation)
 

@@ -137,13 +137,14 @@ int fhoad_adamw_decode(const uint8_t* codes, const float* scales, float* moments
  * 16-byte aligned, that keep g and u in float32 for the backward. workspace:
  * fhoad_gated_linear_forward_workspace_size bytes, 16-byte aligned (NULL when that is 0).
  * float32 products are formed on the 16-bit matrix cores from split operands with float32
- * accumulation, at float32 precision: exactly, as three bf16 parts, or, where that is faster, as
- * two float16 parts of rows scaled to their largest value, with errors of 2^-23 of a value or
- * 2^-51 of its row's largest, whichever is more (a row runs along the contraction: of x and of the
- * weights, in the backward of the gradients and columns that are contracted). bfloat16 products
- * are formed directly. All tensors of one type, with their elements' alignment. rows == 0 enqueues
- * nothing. What follows from an infinite or NaN operand is non-finite, NaN where float32 arithmetic
- * may give an infinity.
+ * accumulation. Smaller layers take three bf16 parts of a value, which hold it but for 2^-126, and
+ * products of them that are good to 2^-24. Larger layers take two float16 parts of rows scaled to
+ * their largest value: errors of 2^-23 of a value or 2^-51 of its row's largest, whichever is more,
+ * and of 2^-22 of a product beside it (a row runs along the contraction: of x and of the weights,
+ * in the backward of the gradients and columns that are contracted). bfloat16 products are formed
+ * directly. All tensors of one type, with their elements' alignment. rows == 0 enqueues nothing.
+ * Projections and gradients formed from an infinite or NaN operand are non-finite, NaN where float32
+ * arithmetic may give an infinity.
  */
 size_t fhoad_gated_linear_saved_size(int64_t rows, int64_t hidden);
 size_t fhoad_gated_linear_forward_workspace_size(int64_t rows, int64_t width, int64_t hidden,

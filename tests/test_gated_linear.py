@@ -536,3 +536,23 @@ def test_the_largest_float32_values(rows, width, hidden) -> None:
     close(run(x * small, with_edges(w.clone()), upstream * small)[1], upstream * small, with_edges(w.clone()))
     close(run(x * small, w * small, with_edges(upstream.clone()))[2], with_edges(upstream.clone()).t(), x * small)
     close(run(with_edges(x.clone()), w * small, upstream * small)[2], upstream.t() * small, with_edges(x.clone()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows, width, hidden", [(5, 64, 70), (64, 64, 70), (600, 40, 700), (700, 2048, 1700),
+                                                 (4000, 520, 1700)])
+def test_operands_whose_low_parts_are_largest(rows, width, hidden) -> None:
+    """Operands of 1 + 2^-11, halfway between two float16 values, where the product of the low parts that the
+    larger layers leave out is largest and of one sign: the products, 1 + 2^-10 + 2^-22, are good to 2^-21
+    and their sums, of equal terms, to that and eight roundings of 2^-24. The gate is tanh(30), one, so h is
+    x Wu^T, the input's gradient dh Wu and the up weights' gradient dh^T x."""
+    require_gpu_extension()
+    show(f"low parts {rows} x {width} x {hidden}")
+    value = 1.0 + 2.0**-11
+    x, up_weight = leaf(torch.full((rows, width), value, device="cuda")), leaf(torch.full((hidden, width), -value, device="cuda"))
+    gate_bias = torch.full((hidden,), 30.0, device="cuda")
+    h = fused_hoad.gated_linear(x, torch.zeros_like(up_weight), up_weight, gate_bias, activation="tanh")
+    dx, dw = torch.autograd.grad(h, (x, up_weight), torch.full_like(h, value))
+    for got, count, sign in ((h, width, -1), (dx, hidden, -1), (dw, rows, 1)):
+        want = sign * count * value * value
+        assert float((got.double() - want).abs().max()) <= (2.0**-21 + 8 * 2.0**-24) * abs(want)
