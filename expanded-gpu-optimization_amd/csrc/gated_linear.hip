@@ -11,7 +11,8 @@
 // six products, or for the larger layers, after a pass that finds each row's scale, into two float16
 // parts and three products (see the formats below): a sixth or a third of the bf16 rate, against a
 // sixteenth with the float32 matrix instructions. bfloat16 operands are used as they are; dg and du
-// are then rounded to bfloat16 once, as operands, which costs what the rounding of the result costs.
+// are then rounded to bfloat16 once, as operands: the gradients' error is 0.0023 of their norm where the
+// results' own rounding makes 0.0017, and in two parts each would double the products' time.
 //
 // 4 rows width hidden operations forward and twice that backward: but for the smallest batches
 // the matrix cores bound it.
@@ -1050,9 +1051,9 @@ __global__ __launch_bounds__(kWaves * kWave) void gated_few_rows_kernel(ForwardA
 // memory straight into operands (each wave splits what it multiplies, so nothing is split once for
 // several), so the chain is an eighth as long; their sums meet in LDS once at the end. Measured, this
 // kernel, the 64 x 64 tiles of Bf16Parts, those of HalfParts without their scales' two launches, us:
-// 64 x 256 x 683 (44 workgroups) 8.9, 17.5, 12.3; 100 x 1,024 x 1,024 (128) 22.1, 50.9, 31.7;
-// 128 x 2,048 x 2,048 (256) 43, 97, 59; with more than a workgroup a CU no longer: 256 x 512 x 1,365
-// (344) 25.1, 28.9, 19.3; 1,000 x 512 x 1,365 (1,376) 65, 38, 24.
+// 64 x 256 x 683 (44 workgroups) 8.0, 17.8, 12.2; 100 x 1,024 x 1,024 (128) 20.0, 52.4, 31.7;
+// 128 x 2,048 x 2,048 (256) 38.9, 99.7, 58.2; 256 x 512 x 1,365 (344) 22.5, 29.6, 18.9; 1,000 x 512 x
+// 1,365 (1,376) 59.4, 41.2, 24.4. It is taken up to a workgroup a CU; the gain ends above that.
 constexpr int kShortWaves = 8, kShortSide = 32;
 
 __device__ __forceinline__ void load_eight(f4 (&v)[2], const float* row, int64_t k, int64_t width) {
@@ -1499,7 +1500,7 @@ int zero(void* out, int64_t n, int dtype, hipStream_t stream) {
 
 // ---- host -------------------------------------------------------------------------------------
 
-constexpr int kCus = 256;
+constexpr int kCus = 256;  // MI355X; on a device of fewer a plan is right as well, and less near the fastest
 constexpr int64_t kPad = 64;  // features to a multiple of every tile's depth
 int64_t padded(int64_t hidden) { return ceil_div(hidden, kPad) * kPad; }
 
@@ -1587,9 +1588,10 @@ Shape shape_of(TileSize size) {
 // it for their first loads and last stores; one alone on its CU takes `alone` of the time it takes
 // among others. What the estimate decides is how the last, partly filled round weighs against the
 // lower rates of smaller tiles, and, where a depth may be cut, against the partial results' bytes.
-// The float32 figures are fitted to 950 measured products of 16 layers (64 to 65,536 rows, 128 to 4,096
-// wide, 93 to 10,240 hidden), which they give to 15 % rms; what the plan takes is 1.2 % from the fastest
-// tile and runs in the geometric mean and 22 % at most.
+// The float32 figures are fitted. Over 1,486 measured products of 18 layers (64 to 65,536 rows, 128 to 4,096
+// wide, 93 to 10,240 hidden) they give the time to 19 % rms, and what the plan takes is 0.6 % from the fastest
+// tile and runs in the geometric mean and 7 % at most. The bfloat16 figures are large products' rates with one
+// common round: over 742 products of these layers 29 % rms, and 8 % from the fastest, 92 % at most.
 struct TileRate {
   int resident;
   double rate, alone, round;

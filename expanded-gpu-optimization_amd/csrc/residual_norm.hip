@@ -6,14 +6,16 @@
 //   t = grad_hidden + rstd (d - xhat mean(d xhat) - mean(d))        (the last term: layer norm)
 //   grad_residual = scale t,  grad_gate = sum of t n,  dn = t gate
 //   grad_block = the same form as t's second term, of dn through the first norm
-// and the weights' gradients are sums over the rows. Every element is read and written once: the
-// forward moves 4 values an element (residual, block in; hidden, normed out), the backward 6, and
-// some 40 float operations each way stay far below the memory's time.
+// and the weights' gradients are sums over the rows. The forward moves 4 values an element (residual,
+// block in; hidden, normed out), the backward 6, and some 40 float operations each way stay far below
+// the memory's time.
 //
 // A row is held in registers by one wave (up to 512 or 1,024 values) or by one workgroup, so the two
-// norms need no second read. The backward forms hidden again from residual and block: the same
-// bytes as reading it, and with bfloat16 without its rounding. Column sums stay in registers over
-// all rows of a workgroup and meet in a second, small launch in a fixed order.
+// norms need no second read; only the backward of rows above 8,192 columns reads a row again in each of
+// its passes, from the caches. The backward forms hidden again from residual and block: the same
+// bytes as reading it, and with bfloat16 without its rounding. Column sums stay with their threads over
+// all rows of a workgroup, in registers (above 4,096 columns some of them in LDS), and meet in a second,
+// small launch in a fixed order.
 #include "network_common.h"
 
 #include <algorithm>
