@@ -186,10 +186,11 @@ class FusedAdamW(torch.optim.Optimizer):
         for p, views in every.items():
             given = states.get(p, {})
             for name, view in views.items():
-                if name in given:
-                    view.copy_(given[name])
-                else:
+                value = given.get(name)
+                if value is None:
                     view.zero_()
+                elif value.data_ptr() != view.data_ptr() or value.dtype != view.dtype:  # not this memory itself
+                    view.copy_(value)
 
     @torch.no_grad()
     def step(self, closure: Callable[[], Tensor] | None = None) -> Tensor | None:
