@@ -353,9 +353,9 @@ __global__ __launch_bounds__(kGroup<kThreads>, (kBackwardWaves<T, kThreads, kWho
   // Above 8,192 columns a thread has 16 values and three sums of each in registers. There, a row's vectors
   // are read one at a time in each of the passes over it, the later times from the caches, and only xhat and
   // the gradient stay between (kReread). 4,882 x 12,288 in us, with all of a row held and now: no norm after
-  // the block, float32 622 and 415 (3.5 TB/s), bfloat16 297 and 190 (3.8); element's gate 1,245 and 546
-  // (4.3), 505 and 351. With a norm after the block and a shared gate five sums still spill: 1,540 and 1,140
-  // (1.3 TB/s), 858 and 836.
+  // the block, float32 622 and 317 (4.5 TB/s), bfloat16 297 and 176 (4.1); element's gate 1,245 and 546
+  // (4.3), 505 and 360. With a norm after the block and a shared gate five sums still spill: 1,540 and 1,120
+  // (1.3 TB/s), 858 and 850.
   constexpr bool kWide = kThreads == 1024;
   constexpr bool kReread = kWide && kPer == 16;
   constexpr int kLdsTotals = !kWide ? 0 : kPer == 8 ? 4 : 2;
@@ -481,7 +481,19 @@ __global__ __launch_bounds__(kGroup<kThreads>, (kBackwardWaves<T, kThreads, kWho
         }
       }
       f2 total = sums(first, second);
-      const float along = total[0] * inverse, level = a.layer ? total[1] * inverse : 0.0f;
+      float along = total[0] * inverse, level = a.layer ? total[1] * inverse : 0.0f, rstd = s[3];
+      // Without grad_normed nothing of the second norm counts, whatever its statistics: they may be
+      // non-finite in a row that the loss leaves out. kClear: its terms are cleared here, otherwise not
+      // selected below. 4,882 x 12,288 float32 and bfloat16 without a norm after the block, in us: cleared 317
+      // and 176, selected 415 and 194; 7,324 x 8,192 with one: 401 and 226, 364 and 209.
+      constexpr bool kClear = kReread && !kPost;
+      if constexpr (kClear) {
+        if (!a.grad_normed) {
+          along = level = rstd = 0.0f;
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) unit_x[e] = grad[e] = 0.0f;
+        }
+      }
       first = second = 0.0f;
       float out[kPer];
 #pragma unroll
@@ -494,7 +506,8 @@ __global__ __launch_bounds__(kGroup<kThreads>, (kBackwardWaves<T, kThreads, kWho
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
           const int e = j * kVec + i;
-          float g = s[3] * (grad[e] - unit_x[e] * along - level);
+          float g = rstd * (grad[e] - unit_x[e] * along - level);
+          if (!kClear && !a.grad_normed) g = 0.0f;
           if (a.grad_hidden) g += to_float(dh[j][i]);
           out[e] = a.scale * g;
           grad[e] = g;
@@ -563,6 +576,10 @@ __global__ __launch_bounds__(kGroup<kThreads>, (kBackwardWaves<T, kThreads, kWho
   if (!a.want_sums) return;
   float* const partials = a.partials + 4 * static_cast<int64_t>(blockIdx.x) * width;
   float sum[kPer];
+  if (!a.grad_normed) {
+    d_weight.clear();
+    d_bias.clear();
+  }
   d_weight.get(sum);
   write_sums<R>(s_row, partials, width, sum);
   d_bias.get(sum);

@@ -447,3 +447,35 @@ def test_rows_of_one_value(kind, gate, unaligned, dtype) -> None:
         want = grads64[name]
         bound = summed(bounds[name], want) + rounding * want.abs()
         assert bool(((grads[name].double() - want).abs() <= bound).all()), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("gate", ["none", "channel", "element"])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("width", [40, 1365, 6001, 12001])
+def test_hidden_alone_with_a_masked_row(width, kind, gate, post, dtype) -> None:
+    """A loss on hidden alone, whose mask leaves out a row that holds an infinity in the residual: nothing goes
+    through the second norm, so the row's gradients are zeros, the other rows' and the sums are finite and
+    as in float64, and the second norm's weight and bias have none."""
+    require_gpu_extension()
+    show(f"residual_norm hidden alone {width} {kind} {gate} post={post} {dtype}")
+    shape = (7, width)
+    t = inputs(shape, dtype, kind, {"none": None, "channel": (width,), "element": shape}[gate], post, kind == "layer", 8)
+    t["residual"][2, width // 2] = math.inf
+    t = {k: leaf(v) for k, v in t.items()}
+    up = normal(*shape, seed=9, dtype=dtype)
+    up[2] = 0
+    wanted = [k for k in NAMES if t[k] is not None]
+    grads = dict(zip(wanted, torch.autograd.grad(call(t, 1.5, kind)[0], [t[k] for k in wanted], up, allow_unused=True)))
+    exact = {k: double(v) for k, v in t.items()}
+    want = dict(zip(wanted, torch.autograd.grad(formula(exact, 1.5, kind, 1e-6)[0], [exact[k] for k in wanted],
+                                                up.double(), allow_unused=True)))
+    for name in wanted:
+        if want[name] is None:
+            assert grads[name] is None or not grads[name].any(), name
+            continue
+        if name in ("residual", "block") or (name == "gate" and gate == "element"):
+            assert not grads[name][2].any(), name
+        assert norm_error(grads[name], want[name]) <= tolerance(dtype, 7 + width), name
