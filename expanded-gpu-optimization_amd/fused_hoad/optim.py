@@ -225,6 +225,10 @@ class FusedAdamW(torch.optim.Optimizer):
         are copied into the packed state with their own types (the base class would cast the moments to
         the parameters' type): into the present one where it has the same layout, else into a new one.
         Nothing is changed when something does not fit."""
+        state_dict = dict(state_dict)  # a hook may change it
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            given = hook(self, state_dict)
+            state_dict = state_dict if given is None else given
         saved = state_dict["param_groups"]
         if [len(g["params"]) for g in saved] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("the state's parameter groups do not match the optimizer's")
@@ -249,6 +253,8 @@ class FusedAdamW(torch.optim.Optimizer):
         for _, views, _ in fills:
             self.state.update(views)
         self._seen = self._tensors()
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
 
     def moments(self, parameter: Tensor) -> tuple[Tensor, Tensor]:
         """``parameter``'s first and second moments in float32 and its shape."""

@@ -728,3 +728,26 @@ def test_last_blocks_of_a_large_tensor() -> None:
         if step == 1:
             assert bool((parameter.detach() == p[0]).all()) and float(p[0]) < 1.0 - 0.9 * OPTIONS["lr"]
         mean, square = decode(codes[0], codes[1], 3), decode(codes[2], codes[3], 4) ** 2
+
+
+def test_hooks_of_load_state_dict_run() -> None:
+    """A hook before the load may give another state, and one after it sees the loaded options."""
+    def build(lr):
+        return fused_hoad.FusedAdamW([torch.nn.Parameter(torch.zeros(3))], lr=lr)
+
+    seen = []
+
+    def before(optimizer, state_dict):
+        seen.append(("before", optimizer.param_groups[0]["lr"]))
+        groups = [{**group, "lr": 2 * group["lr"]} for group in state_dict["param_groups"]]
+        return {**state_dict, "param_groups": groups}
+
+    optimizer = build(0.5)
+    optimizer.register_load_state_dict_pre_hook(lambda o, s: seen.append("first"))
+    optimizer.register_load_state_dict_pre_hook(before)
+    handle = optimizer.register_load_state_dict_post_hook(lambda o: seen.append(("after", o.param_groups[0]["lr"])))
+    optimizer.load_state_dict(build(0.25).state_dict())
+    assert seen == ["first", ("before", 0.5), ("after", 0.5)]
+    handle.remove()
+    optimizer.load_state_dict(build(1.0).state_dict())
+    assert optimizer.param_groups[0]["lr"] == 2.0 and len(seen) == 5
